@@ -676,10 +676,13 @@ int lfm3_prompt_attention_half(const float* q, uint32_t ldq, const uint16_t* k,
  * The structures and the arrays that a call names as host arrays are read
  * before it returns; every pointer in them is device memory, read when the
  * work runs. Rows of queries and outputs are LFM3_TYPE_F32, or have the
- * pages' own type. With FP32 rows the products keep FP32's accuracy (each
- * query and probability enters the matrix cores in parts that add up to it);
- * with 16-bit rows queries enter as they are and a probability rounds to
- * that type once. Scores, maxima, sums and the accumulated weights are FP32.
+ * pages' own type. With FP32 rows each query and probability enters the matrix
+ * cores in parts that add up to it: a query's values to 2^-21 of its row's
+ * largest, a probability to 2^-21 of itself. With 16-bit rows queries enter as
+ * they are and a probability rounds to that type once. (Over F16 pages, either
+ * way, a probability below 2^-29 of the row's largest, or 2^-18 with FP32 rows,
+ * is kept to 2^-40 of the largest.) Scores, maxima, sums and the accumulated
+ * weights are FP32.
  * k, v and weight are 16-byte aligned; dim 64 or 128; page 16, 32, 64, 128
  * or 256; heads a multiple of kv_heads with a group of at most 64; lengths up
  * to 2^30, rows below 2^25.

@@ -40,11 +40,14 @@
 // maximum, the sum and the scale; PagedMergeKernel adds a row's records in
 // span order.
 //
-// FP32 rows: query rows enter in parts (Query), and a probability (F16: times
-// 2^15, so that its second part stays normal) in as many of its type. Rows of
-// the pages' type enter whole; a probability rounds to that type once, by no
-// more than the output itself will. The sum adds the FP32 values in both, for
-// the rows' lse.
+// FP32 rows: query rows enter in parts (Query), and a probability in as many of
+// its type. Rows of the pages' type enter whole; a probability rounds to that
+// type once. F16 probabilities, of either rows, are taken times 2^15: those down
+// to 2^-29 of the column's largest are normal values (rounded by 2^-11 of
+// themselves, no more than the output will be; two parts by 2^-22 down to 2^-18),
+// and none is off by more than 2^-40 of the largest. Unscaled, a long tail of
+// slots e^-17 below a first slot without a value lost a third of the output. The
+// sum adds the FP32 values in both, for the rows' lse.
 #include <algorithm>
 #include <cmath>
 #include <new>
@@ -108,12 +111,13 @@ struct Columns {
   static constexpr bool kHalf = T::kType == LFM3_TYPE_F16;
   static constexpr int kParts = Query<D, T, kRows32>::kParts;
   static constexpr int kSteps = D / 32, kDims = D / 16;
-  static constexpr float kPScale = kRows32 && kHalf ? 32768.0f : 1.0f;
+  static constexpr float kPScale = kHalf ? 32768.0f : 1.0f;  // of probabilities and outputs
+  static constexpr float kPLog2 = kHalf ? 15.0f : 0.0f;
 
   V8 q[CT][kParts][kSteps];
   float scale[CT];  // of raw scores, in units of the natural logarithm
   f4 acc[CT][kDims];
-  float m[CT], l[CT];  // l: the lane's own slots
+  float m[CT], l[CT];  // l: the lane's own slots (16-bit rows: of scaled probabilities)
   int lo[CT], hi[CT];  // slots that the column sees in the span, inclusive
 
   // The wave's columns begin at column `first` of the item.
@@ -200,7 +204,8 @@ struct Columns {
               rest = f2{rest[0] - float(r[0]), rest[1] - float(r[1])};
             }
           } else {
-            const float base2 = -shift * c;
+            // The scale by way of the exponent; Sum() takes it out again.
+            const float base2 = fmaf(-shift, c, kPLog2);
             const f2 e = {__builtin_amdgcn_exp2f(fmaf(s0, c, base2)),
                           __builtin_amdgcn_exp2f(fmaf(s1, c, base2))};
             local[0] += e[0];
@@ -224,6 +229,11 @@ struct Columns {
           p[ct][part][c2] = Pack4<V8>(x);
         }
     }
+  }
+
+  // A column's sum of probabilities, in all its lanes.
+  __device__ __forceinline__ float Sum(int ct) const {
+    return SumXor32(SumXor16(l[ct])) * (kRows32 ? 1.0f : 1.0f / kPScale);
   }
 
   // V^T operand: dimension 16 d + L % 16, slots 32 c2 + 4 (L / 16) + 0..3 and
@@ -472,7 +482,7 @@ __device__ __forceinline__ void NarrowItem(const AttentionArgs& a, const lfm3_pa
   float* s_m = s_acc + kWaves * 16 * kPitch;
   float* s_l = s_m + kWaves * 16;
   const int col = lane & 15, grp = lane >> 4;
-  const float total = SumXor32(SumXor16(cols.l[0]));
+  const float total = cols.Sum(0);
 #pragma unroll
   for (int d = 0; d < Cols::kDims; ++d)
     *reinterpret_cast<f4*>(&s_acc[(wave * 16 + col) * kPitch + 16 * d + 4 * grp]) =
@@ -606,7 +616,7 @@ __device__ __forceinline__ void WideItem(const AttentionArgs& a, const lfm3_page
   const int grp = lane >> 4;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
-    const float l = SumXor32(SumXor16(cols.l[ct]));
+    const float l = cols.Sum(ct);
     const unsigned c = unsigned(c0 + 16 * ct + (lane & 15)), r = c / unsigned(group);
     if (r >= it.rows)
       continue;
