@@ -179,6 +179,20 @@ struct Columns {
       const float shift = next == -INFINITY ? 0.0f : next, c = scale[ct] * kLog2e;
       const float alpha = __builtin_amdgcn_exp2f((m[ct] - shift) * c);
       m[ct] = next;
+      // 16-bit rows: one multiply-add a score, s c - shift c, whose constant rounds
+      // by as much as a score itself does. Where that could pass 2^-4 (the largest
+      // probability would be 2^it, past F16's range or nothing at scores of 10^8),
+      // the shift is taken off first, as FP32 rows always do. The probability's
+      // scale comes by way of the exponent too; Sum() takes it out again.
+      float base2 = fmaf(-shift, c, kPLog2);
+      if constexpr (!kRows32) {
+        if (__ballot(fabsf(base2) >= 0x1p20f)) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+            s[ct][kb] -= shift;
+          base2 = kPLog2;
+        }
+      }
       typedef float f2 __attribute__((ext_vector_type(2)));
       typedef _Float16 e2 __attribute__((ext_vector_type(2)));
       typedef __bf16 b2 __attribute__((ext_vector_type(2)));
@@ -204,8 +218,6 @@ struct Columns {
               rest = f2{rest[0] - float(r[0]), rest[1] - float(r[1])};
             }
           } else {
-            // The scale by way of the exponent; Sum() takes it out again.
-            const float base2 = fmaf(-shift, c, kPLog2);
             const f2 e = {__builtin_amdgcn_exp2f(fmaf(s0, c, base2)),
                           __builtin_amdgcn_exp2f(fmaf(s1, c, base2))};
             local[0] += e[0];

@@ -1,6 +1,6 @@
 """The paged cache's operators at the edges of their types and arguments:
-probabilities far below the largest. Bounds as in paged_util, or derived beside
-the test."""
+probabilities far below the largest, scores that leave one slot. Bounds as in
+paged_util, or derived beside the test."""
 import numpy as np
 import pytest
 
@@ -57,3 +57,54 @@ def test_attention_sink_and_long_tail(gap, heads, kv, dim, columns, span, kind, 
     far = np.abs(got - want) - tol
     worst = np.unravel_index(np.argmax(far), far.shape)
     assert not (far > 0).any(), (worst, got[worst], want[worst], tol[worst])
+
+
+@pytest.mark.parametrize("kind,row_kind,key,query", [
+    (*pair, *size) for pair in PAIRS
+    for size in ((4.0, 20.0), (300.0, 500.0), (3000.0, 30000.0), (3000.0, 3e9))
+    if size[1] < 65504 or pair[1] != F16])
+@pytest.mark.parametrize("columns,span", TILINGS)
+@pytest.mark.parametrize("heads,kv,dim", [(16, 4, 128), (8, 4, 64)])
+def test_attention_of_one_winner(key, query, heads, kv, dim, columns, span, kind, row_kind):
+    """Keys of random signs and a query along one of them: its score is hundreds
+    to 10^14 above every other, the output is its value and lse its score."""
+    pool, b = seeded(211, kv, 32, dim, kind, [40, 1], [700, 500])
+    rng = np.random.default_rng(212)
+    sign = rng.choice(np.array([-1, 1], np.float32), pool.shape)
+    pool.k = P.to_bits(key * sign, kind)
+    q = np.zeros((b.rows, heads, dim), np.float32)
+    want, value = np.zeros(q.shape), P.from_bits(pool.v, kind)
+    for s in range(b.seqs):
+        before = int(b.lengths[s]) - b.counts[s]
+        for j in range(b.counts[s]):
+            r = int(b.starts[s]) + j
+            for h in range(heads):
+                t = int(rng.integers(0, before + j + 1))
+                at = (int(b.table[s, t // 32]), h // (heads // kv), t % 32)
+                q[r, h], want[r, h] = query * sign[at], value[at]
+    pool.upload(), b.upload()
+    gate = rng.standard_normal((b.rows, heads), np.float32)
+    call = P.AttentionCall(pool, b, q, heads, 0, gate, row_kind,
+                           items=P.tiled(b, heads, kv, 0, columns, span))
+    call.launch()
+    L.synchronize()
+    raw, lse = call.results()
+    k0, q0 = np.abs(P.from_bits(pool.k, kind)).max(), np.abs(call.q.values).max()
+    score = k0 * q0 * np.sqrt(dim)
+    # The next largest score: each row's other keys, in units of the winner's.
+    for s in range(b.seqs):
+        page, off, _ = P.slots_of(pool, b.table[s], int(b.lengths[s]))
+        rows = slice(int(b.starts[s]), int(b.starts[s + 1]))
+        for g in range(kv):
+            unit = np.sign(q[rows, g * (heads // kv):(g + 1) * (heads // kv)])
+            second = np.sort((unit @ sign[page, g, off].T / dim), -1)[..., -2].max()
+            assert score * (1 - second) > 40
+    want = want / (1 + np.exp(-gate.astype(np.float64)))[:, :, None]
+    # The probability's rounding (FP32 rows: its parts, 2^-21) and the output's.
+    step = P.HALF_STEP[row_kind]
+    # F16 values below 2^-14 lie 2^-24 apart: half of that.
+    tol = np.abs(want) * (2 * step + 2.0 ** -20) + 2.0 ** -25 * (row_kind == F16)
+    got = raw.reshape(q.shape)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all()
+    # FP32 sums of dim terms of one sign, and the scale's rounding.
+    assert np.abs(lse - score).max() <= score * (dim + 8) * 2.0 ** -24
