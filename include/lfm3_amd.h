@@ -662,8 +662,8 @@ int lfm3_prompt_attention_half(const float* q, uint32_t ldq, const uint16_t* k,
  * slot received are summed into. Sequence s owns the slots [0, lengths[s]);
  * slot t lies at offset t % page of page tables[s * table_stride + t /
  * page]. A table entry that names no page (>= pages, e.g. 0xffffffff) leaves
- * its slots out: nothing is stored to them, no row sees them, eviction ranks
- * them last. Two sequences may share pages that no call writes.
+ * its slots out: nothing is stored to them, no row sees them, eviction drops
+ * them. Two sequences may share pages that no call writes.
  *
  * A batch packs the new rows of its sequences: sequence s has rows
  * starts[s] .. starts[s + 1] - 1 (none where they are equal), which take its
@@ -790,17 +790,20 @@ int lfm3_paged_attention(const lfm3_paged_cache* cache, const lfm3_paged_batch* 
 int lfm3_paged_weights(const lfm3_paged_cache* cache, const lfm3_paged_batch* batch,
                        const void* q, uint32_t ldq, uint32_t row_type, const float* lse,
                        uint32_t heads, uint32_t window, uint32_t max_length, void* stream);
-/* Eviction by accumulated weight. Each KV head of sequence s keeps
-   min(lengths[s], budget) of its slots: the first `sinks`, the last `recent`
-   and, of the others, those of the largest weight (ties toward the lower
-   slot; NaN ranks highest, slots on no page lowest). The kept slots' K, V
-   and weights move, in slot order, to slots 0, 1, ... of new_tables (same
+/* Eviction by accumulated weight. Each KV head of sequence s keeps n of its
+   slots, n = min(those that lie on a page, budget): the first `sinks`, the last
+   `recent` and, of the others that lie on a page, those of the largest weight
+   (ties toward the lower slot; NaN ranks highest). The kept slots' K, V and
+   weights move, in slot order, to slots 0, 1, ... n - 1 of new_tables (same
    layout, new_stride entries a sequence), and their old slot numbers to
-   kept[(s * kv_heads + g) * budget + i]; entries past the number kept, and
-   everything on the old pages, are left as they were. The new tables' pages
-   must not be pages of any old table of the call (shared prefixes stay
-   whole), nor of two new tables. sinks + recent <= budget; max_length: at
-   least every lengths[s] (later slots are left out). */
+   kept[(s * kv_heads + g) * budget + i]. n, the same for every KV head, is the
+   sequence's length on its new table; entries and new slots past it, and
+   everything on the old pages, are left as they were. The sinks and the recent
+   slots have to lie on pages (one that does not counts all the same, and what
+   its new slot holds stays there). The new tables' pages must not be pages of
+   any old table of the call (shared prefixes stay whole), nor of two new
+   tables. sinks + recent <= budget; max_length: at least every lengths[s] (later
+   slots are left out). */
 size_t lfm3_paged_evict_workspace_bytes(uint32_t seqs, uint32_t kv_heads, uint32_t budget,
                                         uint32_t max_length);
 int lfm3_paged_evict(const lfm3_paged_cache* cache, const uint32_t* tables,

@@ -127,8 +127,55 @@ struct EvictArgs {
   const std::uint32_t* lengths;
   std::uint32_t max_length, budget, sinks, recent;
   std::uint32_t* kept;
+  unsigned* counts;  // of each list's kept slots; NULL: the move finds them again
   int kv_heads;
 };
+
+// What a sequence keeps: its first `lo` slots, those from `hi` on, and of those
+// between that lie on a page up to `need`.
+struct EvictRange {
+  std::uint32_t length, lo, hi, need;
+  __device__ __forceinline__ EvictRange(const EvictArgs& a, int seq) {
+    length = min(a.lengths[seq], a.max_length);
+    lo = min(a.sinks, length);
+    hi = max(lo, length - min(a.recent, length));
+    need = a.budget - a.sinks - a.recent;
+  }
+  // Slots kept in all, `ranked` of them between lo and hi.
+  __device__ __forceinline__ std::uint32_t Count(std::uint32_t ranked) const {
+    return lo + ranked + (length - hi);
+  }
+};
+
+// A thread's share of the number of a sequence's slots [from, to) that lie on a
+// page.
+__device__ __forceinline__ unsigned PresentShare(const PageTable& table, int seq,
+                                                 std::uint32_t from, std::uint32_t to,
+                                                 int threads) {
+  unsigned n = 0;
+  if (from < to)
+    for (std::uint32_t e = (from >> table.shift) + threadIdx.x; e <= (to - 1) >> table.shift;
+         e += threads)
+      if (table.Page(seq, e << table.shift) < table.pages)
+        n += min(to, (e + 1) << table.shift) - max(from, e << table.shift);
+  return n;
+}
+// The sum of every thread's v in all threads; s_wave: a word a wave.
+template<int kWaves>
+__device__ __forceinline__ unsigned BlockTotal(unsigned v, unsigned* s_wave) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1)
+    v += __shfl_xor(v, d);
+  if ((threadIdx.x & 63) == 0)
+    s_wave[threadIdx.x >> 6] = v;
+  __syncthreads();
+  unsigned total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    total += s_wave[w];
+  __syncthreads();
+  return total;
+}
 
 // Workspace of an eviction in slices (LaunchSlices).
 struct EvictSlices {
@@ -204,24 +251,35 @@ __device__ __forceinline__ uint2 FindBin(unsigned x0, unsigned x1, unsigned need
   return make_uint2(s_pick[0], s_pick[1]);
 }
 
-// Slots [from, to) of a sequence's `length`, in order, to their places in the
-// kept list: those before `lo` and from `hi` on, of the others those of a rank
-// above `prefix`, and the first `need` of rank `prefix`. above, equal: what of
-// these the slots between lo and `from` hold. The block's waves take a stretch
-// each: they count, exchange the counts, and write.
+// Where the ranked slots are cut: those of a rank above `prefix` are kept and the
+// first `need` of rank `prefix`, `ranked` in all.
+struct Cut {
+  unsigned prefix, need, ranked;
+  // wanted: slots asked for; prefix, need: the last one's rank, and what is
+  // needed of it (nothing of rank 0, which is on no page).
+  static __device__ __forceinline__ Cut At(unsigned wanted, unsigned prefix, unsigned need) {
+    if (!wanted)
+      return Cut{0xffffffffu, 0, 0};
+    return prefix ? Cut{prefix, need, wanted} : Cut{0, 0, wanted - need};
+  }
+  // All that lie on a page, of which there are `present`; their rank is 1.
+  static __device__ __forceinline__ Cut Present(unsigned present) { return Cut{0, 0, present}; }
+};
+
+// Slots [from, to) of a sequence, in order, to their places in the kept list:
+// those before lo and from hi on, and those between that the cut leaves. above,
+// equal: what of its rank and above the slots between lo and `from` hold. The
+// block's waves take a stretch each: they count, exchange the counts, and write.
 template<class Rank>
 __device__ __forceinline__ void WriteKept(std::uint32_t* kept, std::uint32_t from,
-                                          std::uint32_t to, std::uint32_t length,
-                                          std::uint32_t lo, std::uint32_t hi,
-                                          std::uint32_t budget, unsigned prefix, unsigned need,
-                                          unsigned above, unsigned equal, unsigned* s_above,
-                                          unsigned* s_equal, Rank rank) {
+                                          std::uint32_t to, const EvictRange& range,
+                                          const Cut& cut, unsigned above, unsigned equal,
+                                          unsigned* s_above, unsigned* s_equal, Rank rank) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const std::uint32_t stretch =
       ((to - from + kSelectWaves - 1) / kSelectWaves + 63) / 64 * 64;
   const std::uint32_t begin = min(from + wave * stretch, to), end = min(begin + stretch, to);
-  // Ranks of four runs of 64 slots, in flight together. need 0: the threshold
-  // is above every rank.
+  // Ranks of four runs of 64 slots, in flight together.
   constexpr int kRuns = 4;
   struct State {
     bool more, same;
@@ -234,8 +292,8 @@ __device__ __forceinline__ void WriteKept(std::uint32_t* kept, std::uint32_t fro
 #pragma unroll
     for (int j = 0; j < kRuns; ++j) {
       const std::uint32_t t = t0 + 64 * j + lane;
-      const bool ranked = t < end && t >= lo && t < hi && need;
-      x[j] = State{ranked && r[j] > prefix, ranked && r[j] == prefix};
+      const bool ranked = t < end && t >= range.lo && t < range.hi;
+      x[j] = State{ranked && r[j] > cut.prefix, ranked && r[j] == cut.prefix};
     }
   };
   unsigned n_above = 0, n_equal = 0;
@@ -267,12 +325,12 @@ __device__ __forceinline__ void WriteKept(std::uint32_t* kept, std::uint32_t fro
       const unsigned long long all_more = __ballot(x[j].more), all_same = __ballot(x[j].same);
       const unsigned my_above = above + __popcll(all_more & before);
       const unsigned my_equal = equal + __popcll(all_same & before);
-      if (t < end && t < lo)
+      if (t < end && t < range.lo)
         kept[t] = t;
-      else if (t < end && t >= hi)
-        kept[budget - (length - t)] = t;
-      else if (x[j].more || (x[j].same && my_equal < need))
-        kept[lo + my_above + min(my_equal, need)] = t;
+      else if (t < end && t >= range.hi)
+        kept[range.lo + cut.ranked + (t - range.hi)] = t;
+      else if (x[j].more || (x[j].same && my_equal < cut.need))
+        kept[range.lo + my_above + min(my_equal, cut.need)] = t;
       above += __popcll(all_more);
       equal += __popcll(all_same);
     }
@@ -281,41 +339,49 @@ __device__ __forceinline__ void WriteKept(std::uint32_t* kept, std::uint32_t fro
 
 // The slots that KV head g of sequence s keeps, in order, by one block. Where
 // more slots are there than the budget, the rank of the last weight kept is
-// found digit by digit over the slots between `sinks` and `recent`. What bounds
-// it is the chain of its passes (32 lists of 2300 slots take 11 us, of which a
-// launch is 3), not its 0.3 MB.
+// found digit by digit over the slots between `sinks` and `recent`; else all that
+// lie on a page are kept. What bounds it is the chain of its passes (32 lists of
+// 2300 slots take 11 us, of which a launch is 3), not its 0.3 MB.
 __launch_bounds__(kSelectThreads) __global__ void PagedSelectKernel(EvictArgs a) {
   extern __shared__ unsigned s_rank[];
   __shared__ unsigned s_bins[kBins], s_total[kSelectWaves], s_pick[2];
   __shared__ unsigned s_above[kSelectWaves], s_equal[kSelectWaves];
   const int g = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
-  const std::uint32_t length = min(a.lengths[seq], a.max_length);
-  std::uint32_t* kept = a.kept + (std::size_t(seq) * a.kv_heads + g) * a.budget;
-  if (length <= a.budget) {
-    for (std::uint32_t i = tid; i < length; i += kSelectThreads)
-      kept[i] = i;
+  const EvictRange range(a, seq);
+  const std::size_t list = std::size_t(seq) * a.kv_heads + g;
+  std::uint32_t* kept = a.kept + list * a.budget;
+  if (range.length <= a.budget) {
+    const unsigned present = BlockTotal<kSelectWaves>(
+        PresentShare(a.table, seq, range.lo, range.hi, kSelectThreads), s_total);
+    if (a.counts && tid == 0)
+      a.counts[list] = range.Count(present);
+    if (present == range.hi - range.lo) {
+      for (std::uint32_t i = tid; i < range.length; i += kSelectThreads)
+        kept[i] = i;
+      return;
+    }
+    WriteKept(kept, 0, range.length, range, Cut::Present(present), 0, 0, s_above, s_equal,
+              [&](std::uint32_t t) { return a.table.Page(seq, t) < a.table.pages ? 1u : 0u; });
     return;
   }
-  const std::uint32_t lo = a.sinks, hi = length - a.recent;  // ranked slots [lo, hi)
-  unsigned need = a.budget - a.sinks - a.recent;  // of them are kept: fewer than there are
-  unsigned prefix = 0;
+  unsigned need = range.need, prefix = 0;  // fewer than there are
   if (need) {
     // Eight at a time: a page's number, then its weight, are a round trip each.
-    for (std::uint32_t t0 = tid; t0 < length; t0 += 8 * kSelectThreads) {
+    for (std::uint32_t t0 = tid; t0 < range.length; t0 += 8 * kSelectThreads) {
       unsigned r[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        r[j] = ReadRank(a, seq, g, min(t0 + j * kSelectThreads, length - 1));
+        r[j] = ReadRank(a, seq, g, min(t0 + j * kSelectThreads, range.length - 1));
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (t0 + j * kSelectThreads < length)
+        if (t0 + j * kSelectThreads < range.length)
           s_rank[t0 + j * kSelectThreads] = r[j];
     }
     for (int d = 0; d < 3; ++d) {
       const Digit digit(d);
       s_bins[tid] = s_bins[tid + kSelectThreads] = 0;
       __syncthreads();
-      for (std::uint32_t t = lo + tid; t < hi; t += kSelectThreads) {
+      for (std::uint32_t t = range.lo + tid; t < range.hi; t += kSelectThreads) {
         const unsigned r = s_rank[t];
         if ((r & digit.Before()) == prefix)
           atomicAdd(&s_bins[digit.Bin(r)], 1u);
@@ -327,8 +393,8 @@ __launch_bounds__(kSelectThreads) __global__ void PagedSelectKernel(EvictArgs a)
       need = pick.y;
     }
   }
-  WriteKept(kept, 0, length, length, lo, hi, a.budget, prefix, need, 0, 0, s_above, s_equal,
-            [&](std::uint32_t t) { return s_rank[t]; });
+  WriteKept(kept, 0, range.length, range, Cut::At(range.need, prefix, need), 0, 0, s_above,
+            s_equal, [&](std::uint32_t t) { return s_rank[t]; });
 }
 
 // The same in slices of a sequence's slots, a block each, one launch a digit:
@@ -343,19 +409,27 @@ __launch_bounds__(kSelectThreads) __global__ void PagedSliceKernel(EvictArgs a, 
   __shared__ unsigned s_bins[kBins], s_total[kSelectWaves], s_pick[2];
   __shared__ unsigned s_above[kSelectWaves], s_equal[kSelectWaves];
   const int slice = blockIdx.x, g = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x;
-  const std::uint32_t length = min(a.lengths[seq], a.max_length);
+  const EvictRange range(a, seq);
+  const std::uint32_t length = range.length, lo = range.lo, hi = range.hi;
   const std::uint32_t from = std::uint32_t(slice) * w.slice, to = min(from + w.slice, length);
   const std::size_t list = std::size_t(seq) * a.kv_heads + g,
                     lists = std::size_t(gridDim.z) * a.kv_heads;
   std::uint32_t* kept = a.kept + list * a.budget;
   if (length <= a.budget) {
-    if (kDigit == 3)
-      for (std::uint32_t t = from + tid; t < to; t += kSelectThreads)
-        kept[t] = t;
+    if constexpr (kDigit == 3) {
+      const unsigned before = BlockTotal<kSelectWaves>(
+          PresentShare(a.table, seq, lo, min(from, hi), kSelectThreads), s_total);
+      const unsigned present = before + BlockTotal<kSelectWaves>(
+          PresentShare(a.table, seq, max(lo, min(from, hi)), hi, kSelectThreads), s_total);
+      if (slice == 0 && tid == 0)
+        a.counts[list] = range.Count(present);
+      if (from < to)
+        WriteKept(kept, from, to, range, Cut::Present(present), before, 0, s_above, s_equal,
+                  [&](std::uint32_t t) { return a.table.Page(seq, t) < a.table.pages ? 1u : 0u; });
+    }
     return;
   }
-  const std::uint32_t lo = a.sinks, hi = length - a.recent;
-  unsigned need = a.budget - a.sinks - a.recent, prefix = 0, above = 0, equal = 0;
+  unsigned need = range.need, prefix = 0, above = 0, equal = 0;
   unsigned* ranks = w.ranks + list * w.slices * w.slice;
   if (kDigit > 0 && need) {
     const Digit last(kDigit - 1);
@@ -415,9 +489,12 @@ __launch_bounds__(kSelectThreads) __global__ void PagedSliceKernel(EvictArgs a, 
     }
   }
   if constexpr (kDigit == 3) {
+    const Cut cut = Cut::At(range.need, prefix, need);
+    if (slice == 0 && tid == 0)
+      a.counts[list] = range.Count(cut.ranked);
     if (from < to)
-      WriteKept(kept, from, to, length, lo, hi, a.budget, prefix, need, above, equal, s_above,
-                s_equal, [&](std::uint32_t t) { return ranks[t]; });
+      WriteKept(kept, from, to, range, cut, above, equal, s_above, s_equal,
+                [&](std::uint32_t t) { return ranks[t]; });
   } else {
     const Digit digit(kDigit);
     s_bins[tid] = s_bins[tid + kSelectThreads] = 0;
@@ -450,38 +527,56 @@ __launch_bounds__(kSelectThreads) __global__ void PagedSliceKernel(EvictArgs a, 
 
 // The kept slots' rows and weights to the new pages, D / 8 threads a slot, 16
 // bytes each: bound by the copy (32 lists of 2048 slots, 67 MB both ways, 12 us:
-// 5.6 TB/s out of the caches that hold part of it).
+// 5.6 TB/s out of the caches that hold part of it). How many there are is the
+// same for every head; where no count was kept (lists of up to kOneBlock slots)
+// each block adds up the table's pages while its rows are on their way.
 template<int D>
 __launch_bounds__(256) __global__ void PagedMoveKernel(EvictArgs a) {
   constexpr int S = D / 8, kSlots = 256 / S;
+  __shared__ unsigned s_wave[4];
   const int g = blockIdx.y, seq = blockIdx.z, seg = threadIdx.x % S;
-  const std::uint32_t count = min(min(a.lengths[seq], a.max_length), a.budget);
+  const EvictRange range(a, seq);
+  const std::size_t list = std::size_t(seq) * a.kv_heads + g;
+  const std::uint32_t most = min(range.length, a.budget);
+  if (blockIdx.x * kSlots >= most)
+    return;
   const std::uint32_t to = blockIdx.x * kSlots + threadIdx.x / S;
-  if (to >= count)
-    return;
-  const std::uint32_t from = a.kept[(std::size_t(seq) * a.kv_heads + g) * a.budget + to];
+  const std::uint32_t from = a.kept[list * a.budget + min(to, most - 1)];
   const std::uint32_t page = a.table.Page(seq, from), new_page = a.new_table.Page(seq, to);
-  if (page >= a.table.pages || new_page >= a.table.pages)
-    return;
+  // An entry that the list does not have reads some slot or page 0.
   const int page_slots = 1 << a.table.shift;
   const std::size_t src =
-      (std::size_t(page) * a.kv_heads + g) * page_slots + (from & (page_slots - 1));
+      (std::size_t(page < a.table.pages ? page : 0u) * a.kv_heads + g) * page_slots +
+      (from & (page_slots - 1));
   const std::size_t dst =
       (std::size_t(new_page) * a.kv_heads + g) * page_slots + (to & (page_slots - 1));
   const uint4 k = reinterpret_cast<const uint4*>(a.k_pages)[src * S + seg];
   const uint4 v = reinterpret_cast<const uint4*>(a.v_pages)[src * S + seg];
+  const float w = a.weight[src];
+  std::uint32_t count;
+  if (a.counts)
+    count = a.counts[list];
+  else
+    count = range.Count(min(
+        range.need,
+        BlockTotal<4>(PresentShare(a.table, seq, range.lo, range.hi, 256), s_wave)));
+  if (to >= count || page >= a.table.pages || new_page >= a.table.pages)
+    return;
   reinterpret_cast<uint4*>(a.k_pages)[dst * S + seg] = k;
   reinterpret_cast<uint4*>(a.v_pages)[dst * S + seg] = v;
   if (seg == 0)
-    a.weight[dst] = a.weight[src];
+    a.weight[dst] = w;
 }
 
 // The slices of lists of up to max_length slots, and their workspace.
 struct SlicePlan {
   std::uint32_t slice = 0, slices = 0;  // slices 0: one block a list
-  std::size_t ranks = 0, bins = 0, state = 0, above = 0;  // bytes
+  std::size_t ranks = 0, bins = 0, state = 0, above = 0, counts = 0;  // bytes
   SlicePlan(std::size_t lists, std::uint32_t budget, std::uint32_t max_length) {
-    if (max_length <= kOneBlock || max_length <= budget)
+    if (max_length <= kOneBlock)
+      return;
+    counts = lists * sizeof(unsigned);
+    if (max_length <= budget)
       return;
     slice = std::max(kSlice, (max_length + kMaxSlices - 1) / kMaxSlices);
     if (lists * ((max_length + slice - 1) / slice) > kCus)
@@ -492,7 +587,7 @@ struct SlicePlan {
     state = 2 * lists * sizeof(uint2);
     above = lists * slices * sizeof(unsigned);
   }
-  std::size_t Bytes() const { return bins + state + ranks + above; }
+  std::size_t Bytes() const { return bins + state + ranks + above + counts; }
 };
 
 }  // namespace
@@ -572,10 +667,12 @@ int lfm3_paged_evict(const lfm3_paged_cache* cache, const std::uint32_t* tables,
   EvictArgs a{static_cast<Half*>(cache->k), static_cast<Half*>(cache->v), cache->weight,
               PageTable{tables, table_stride, cache->pages, shift},
               PageTable{new_tables, new_stride, cache->pages, shift}, lengths, max_length, budget,
-              sinks, recent, kept, int(cache->kv_heads)};
+              sinks, recent, kept, nullptr, int(cache->kv_heads)};
   const auto s = static_cast<hipStream_t>(stream);
+  char* at = static_cast<char*>(workspace);
+  if (plan.counts)
+    a.counts = reinterpret_cast<unsigned*>(at + plan.Bytes() - plan.counts);
   if (plan.slices) {
-    char* at = static_cast<char*>(workspace);
     EvictSlices w;
     w.bins = reinterpret_cast<unsigned*>(at);
     w.state = reinterpret_cast<uint2*>(at + plan.bins);

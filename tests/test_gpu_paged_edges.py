@@ -1,6 +1,8 @@
 """The paged cache's operators at the edges of their types and arguments:
-probabilities far below the largest, scores that leave one slot. Bounds as in
-paged_util, or derived beside the test."""
+probabilities far below the largest, scores that leave one slot, evictions of
+sequences that miss pages. Bounds as in paged_util, or derived beside the test."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -108,3 +110,97 @@ def test_attention_of_one_winner(key, query, heads, kv, dim, columns, span, kind
     assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all()
     # FP32 sums of dim terms of one sign, and the scale's rounding.
     assert np.abs(lse - score).max() <= score * (dim + 8) * 2.0 ** -24
+
+
+# Sequences: (length, the table entries that name no page). Sinks and recent
+# slots lie on pages, as the call asks.
+MISSING = [
+    # fewer present than the budget; none missing; all but the first and last page
+    (16, 96, 4, 10, [(200, range(1, 9)), (100, []), (160, range(1, 9)), (7, [])]),
+    # a length within the budget, with and without holes; one slot past it
+    (16, 128, 4, 16, [(128, [2, 5]), (90, [1]), (60, []), (129, [3]), (0, [])]),
+    # nothing between the sinks and the recent slots
+    (32, 64, 32, 32, [(640, [3, 9]), (64, []), (40, [])]),
+    # no sinks: the first pages are gone, as a sliding window leaves them
+    (64, 1000, 0, 100, [(3000, range(0, 40)), (900, [0, 1]), (1500, range(0, 20))]),
+    # in slices: too few present, enough, and lengths within the budget
+    (64, 5000, 4, 64, [(20000, range(1, 300)), (20000, range(1, 100)), (4000, [3, 20]),
+                       (300, [])]),
+    # longer than a block's ranks and all within the budget; nothing left of the last
+    (128, 20000, 0, 0, [(18000, [0, 7, 100]), (17000, []), (100, [0])]),
+]
+
+
+@pytest.mark.parametrize("kind,dim", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("shape", range(len(MISSING)))
+def test_evict_drops_slots_on_no_page(shape, kind, dim):
+    """A sequence keeps what lies on a page, up to the budget; what the new pages
+    held before is seen by no row and ranks nowhere afterwards."""
+    page, budget, sinks, recent, sequences = MISSING[shape]
+    kv, heads, n = 2, 4, len(sequences)
+    lengths = [length for length, _ in sequences]
+    counts = [max(-(-length // page), 1) for length in lengths]
+    new_counts = [max(-(-(min(length, budget) + 1) // page), 1) for length in lengths]
+    pool = P.Pool(221, sum(counts) + sum(new_counts) + 1, kv, page, dim, kind)
+    both = P.tables(222, counts + new_counts, pool.pages)
+    table, new = both[:n, :max(counts)].copy(), both[n:, :max(new_counts)].copy()
+    for s, (_, missing) in enumerate(sequences):
+        table[s, list(missing)] = [0xFFFFFFFF, pool.pages, 0x80000000][s % 3]
+    nan = P.to_bits(np.float32(np.nan), kind)
+    fresh = new[new < pool.pages]
+    pool.k[fresh], pool.v[fresh], pool.w[fresh] = nan, nan, np.nan
+    pool.upload()
+    # The call, restated: what is on a page, less the lightest between the ends.
+    old_k, old_v, old_w = pool.k.copy(), pool.v.copy(), pool.w.copy()
+    room = min(budget, max(lengths))
+    kept = np.full((n, kv, budget), 0xABABABAB, np.uint32)
+    left = []
+    for s, length in enumerate(lengths):
+        at, off, present = (x[:length] for x in P.slots_of(pool, table[s], max(length, 1)))
+        t = np.arange(length)
+        always = (t < sinks) | (t + recent >= length)
+        left.append(min(int(present.sum()), budget))
+        for g in range(kv):
+            ranked = t[present & ~always]
+            ranked = ranked[np.argsort(-old_w[at[ranked], g, off[ranked]], kind="stable")]
+            mine = np.sort(np.concatenate([t[always], ranked[:left[s] - always.sum()]]))
+            assert len(mine) == left[s]
+            kept[s, g, :len(mine)] = mine
+            to, to_off, _ = P.slots_of(pool, new[s], max(len(mine), 1))
+            to, to_off = to[:len(mine)], to_off[:len(mine)]
+            for x, old in ((pool.k, old_k), (pool.v, old_v), (pool.w, old_w)):
+                x[to, g, to_off] = old[at[mine], g, off[mine]]
+    assert room <= new.shape[1] * page
+    dt, dn, dl = (L.DeviceBuffer.of(np.ascontiguousarray(x, np.uint32))
+                  for x in (table, new, lengths))
+    out = L.DeviceBuffer.of(np.full(kept.size, 0xABABABAB, np.uint32))
+    need = L.lib().lfm3_paged_evict_workspace_bytes(n, kv, budget, max(lengths))
+    ws = L.DeviceBuffer.of(np.full(max(need, 16), 0x5A, np.uint8))
+    L.check(L.lib().lfm3_paged_evict(
+        C.byref(pool.cache), dt.addr, table.shape[1], dl.addr, n, max(lengths), dn.addr,
+        new.shape[1], budget, sinks, recent, out.addr, ws.addr, need, None))
+    L.synchronize()
+    assert np.array_equal(out.download(np.uint32, kept.size).reshape(kept.shape), kept)
+    gk, gv, gw = pool.download()
+    assert np.array_equal(gk, pool.k) and np.array_equal(gv, pool.v)
+    assert np.array_equal(gw.view(np.uint32), pool.w.view(np.uint32))
+    # One more token a sequence: heads, attention and weights on the new table.
+    b = P.Batch([1] * n, np.array(left) + 1, new).upload()
+    rng = np.random.default_rng(223)
+    call = P.AttentionCall(pool, b, rng.standard_normal((n, heads, dim), np.float32), heads, 0)
+    x = L.DeviceBuffer.of(rng.standard_normal((n, heads * dim), np.float32))
+    ones = L.DeviceBuffer.of(np.ones(dim, np.float32))
+    L.check(L.lib().lfm3_paged_heads(
+        C.byref(pool.cache), C.byref(b.batch), call.q.addr, x.addr, x.addr, heads * dim,
+        ones.addr, ones.addr, ones.addr, None, call.q.addr, call.q.ld, F32, heads, 1e-5, None))
+    call.launch()
+    L.check(L.lib().lfm3_paged_weights(
+        C.byref(pool.cache), C.byref(b.batch), call.q.addr, call.q.ld, F32, call.lse.addr, heads,
+        0, max(left) + 1, None))
+    L.synchronize()
+    pool.k, pool.v, gw = pool.download()
+    call.q.values = call.q.download().reshape(n, heads, dim)
+    P.check_attention(call, shape)
+    for s in range(n):
+        at, off, _ = P.slots_of(pool, new[s], left[s] + 1)
+        assert np.isfinite(gw[at, :, off]).all()
