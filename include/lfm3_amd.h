@@ -785,8 +785,9 @@ int lfm3_paged_attention(const lfm3_paged_cache* cache, const lfm3_paged_batch* 
    the slot (as in lfm3_paged_attention, whose q and lse these are; a row
    whose lse is -inf gives nothing). No atomics: the sums' order is fixed, and
    sequences of one call must not share pages (their weights are written).
-   max_length: at least every lengths[s] (host bound of the grid; later slots
-   are left out). */
+   max_length: at least every lengths[s] (later slots are left out); times
+   kv_heads and, up to 64, seqs it stays below 2^40 (max_length rounded up to
+   512; refused beyond). */
 int lfm3_paged_weights(const lfm3_paged_cache* cache, const lfm3_paged_batch* batch,
                        const void* q, uint32_t ldq, uint32_t row_type, const float* lse,
                        uint32_t heads, uint32_t window, uint32_t max_length, void* stream);

@@ -34,6 +34,7 @@ constexpr std::uint32_t kBlocks = 256;
 // Decode rows' turns a block up to which it takes them from one list, and the
 // blocks that these are reckoned for (every list rounds up).
 constexpr int kFewTurns = 4, kNarrowUnits = 224;
+constexpr std::uint64_t kMaxUnits = 0x7fffffff, kUnitSlots = std::uint64_t(kWaves) * kWideSlots;
 constexpr std::size_t kNarrowLds = std::size_t(kWaves) * 16384;
 constexpr float kLog2e = 1.44269504088896341f;
 
@@ -129,7 +130,8 @@ __device__ __forceinline__ Work CountUnits(const WeightsArgs& a, int group, int 
 }
 
 // Unit `at` of the batch's units of a shape, lists in order of (sequence, KV
-// head).
+// head). Sums over 64 sequences fit 32 bits (kMaxUnits; a unit of a shape that is
+// looked for here has 512 slots at least, or there are kBlocks of them at most).
 template<bool kNarrow>
 __device__ __forceinline__ Unit FindUnit(const WeightsArgs& a, long long at, int group, int size,
                                          int lane) {
@@ -563,6 +565,7 @@ __launch_bounds__(64 * kWaves, 2) __global__ void PagedWeightsKernel(WeightsArgs
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int group = a.heads / a.kv_heads, lane = threadIdx.x & 63;
   constexpr int kTurn = kWaves * 8192 / D;  // slots that the waves' stages hold
+  static_assert(kTurn >= int(kUnitSlots), "the host's bound of the units");
   const Work work = CountUnits(a, group, kTurn, lane);
   const long long turns = work.turns;
   const int few = int(min((turns + kNarrowUnits - 1) / kNarrowUnits, 1ll << 20));
@@ -582,6 +585,8 @@ __launch_bounds__(64 * kWaves, 2) __global__ void PagedWeightsKernel(WeightsArgs
     const long long last = turns * (blockIdx.x + 1) / gridDim.x;
     for (long long at = turns * blockIdx.x / gridDim.x; at < last;) {
       const Unit unit = FindUnit<true>(a, at, group, kTurn, lane);
+      if (!unit.count)
+        break;
       const int n = int(min(last - at, (long long)(unit.count - unit.index)));
       const int begin = unit.rows.from + unit.index * kTurn;
       NarrowSlots<D, T, kRows32>(a, unit, begin, min(begin + n * kTurn, unit.rows.length), group,
@@ -591,6 +596,8 @@ __launch_bounds__(64 * kWaves, 2) __global__ void PagedWeightsKernel(WeightsArgs
   }
   for (long long at = blockIdx.x; at < work.wide; at += gridDim.x) {
     const Unit unit = FindUnit<false>(a, at, group, work.shares, lane);
+    if (!unit.count)
+      break;
     if (Shares(unit.rows.rows * group, work.shares) > 2)
       WideUnit<D, T, kRows32, true>(a, unit, group, work.shares, lds);
     else
@@ -640,6 +647,9 @@ extern "C" int lfm3_paged_weights(const lfm3_paged_cache* cache, const lfm3_page
                                                    kMaxLength));
   if (!batch->rows || !max_length)
     return LFM3_OK;
+  if (std::uint64_t(std::min(batch->seqs, 64u)) * cache->kv_heads *
+          ((max_length + kUnitSlots - 1) / kUnitSlots) > kMaxUnits)
+    return Fail(LFM3_E_INVALID, "LFM3 paged weights: too many slots");
   const WeightsArgs a{q, ldq, lse, static_cast<const Half*>(cache->k), cache->weight,
                       PageTable{batch->tables, batch->table_stride, cache->pages,
                                 PageShift(cache->page)},
