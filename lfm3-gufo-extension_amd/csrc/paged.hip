@@ -22,6 +22,7 @@ struct HeadsArgs {
   const std::uint32_t *starts, *lengths, *positions;
   int seqs, heads, kv_heads;
   float eps;
+  std::uint32_t first_row;  // of the launch
 };
 
 // The sequence of a row: the number of starts[1 ..] at or before it. Lanes
@@ -53,7 +54,7 @@ template<int D, class T, bool kRows32>
 __launch_bounds__(256) __global__ void PagedHeadsKernel(HeadsArgs a) {
   constexpr int P = D / 2, kParts = 256 / P;
   const int tid = threadIdx.x, pair = tid % P, part = tid / P;
-  const std::uint32_t row = blockIdx.x;
+  const std::uint32_t row = a.first_row + blockIdx.x;
   const int seq = SequenceOf(a.starts, a.seqs, row, tid & 63);
   if (seq >= a.seqs || row < a.starts[seq])
     return;
@@ -101,12 +102,20 @@ __launch_bounds__(256) __global__ void PagedHeadsKernel(HeadsArgs a) {
   }
 }
 
+// Blocks of a launch in x: a grid has less than 2^32 threads there.
+constexpr std::uint32_t kMaxBlocks = 1u << 23;
+
 template<int D, class T>
-void LaunchHeads(const HeadsArgs& a, dim3 grid, bool rows32, hipStream_t s) {
-  if (rows32)
-    PagedHeadsKernel<D, T, true><<<grid, 256, 0, s>>>(a);
-  else
-    PagedHeadsKernel<D, T, false><<<grid, 256, 0, s>>>(a);
+void LaunchHeads(HeadsArgs a, std::uint32_t rows, std::uint32_t units, bool rows32,
+                 hipStream_t s) {
+  constexpr std::uint32_t kParts = 512 / D;
+  for (; a.first_row < rows; a.first_row += kMaxBlocks) {
+    const dim3 grid(std::min(rows - a.first_row, kMaxBlocks), (units + kParts - 1) / kParts);
+    if (rows32)
+      PagedHeadsKernel<D, T, true><<<grid, 256, 0, s>>>(a);
+    else
+      PagedHeadsKernel<D, T, false><<<grid, 256, 0, s>>>(a);
+  }
 }
 
 // ------------------------------------------------------------------- evict
@@ -621,17 +630,16 @@ int lfm3_paged_heads(const lfm3_paged_cache* cache, const lfm3_paged_batch* batc
               static_cast<Half*>(cache->k), static_cast<Half*>(cache->v), cache->weight,
               PageTable{batch->tables, batch->table_stride, cache->pages, PageShift(cache->page)},
               batch->starts, batch->lengths, batch->positions, int(batch->seqs), int(heads),
-              int(cache->kv_heads), eps};
-  const std::uint32_t parts = 512 / cache->dim, units = heads + 2 * cache->kv_heads;
-  const dim3 grid(batch->rows, (units + parts - 1) / parts);
+              int(cache->kv_heads), eps, 0};
+  const std::uint32_t rows = batch->rows, units = heads + 2 * cache->kv_heads;
   const auto s = static_cast<hipStream_t>(stream);
   const bool rows32 = row_type == LFM3_TYPE_F32, half = cache->type == LFM3_TYPE_F16;
   if (cache->dim == 128)
-    half ? LaunchHeads<128, F16Pages>(a, grid, rows32, s)
-         : LaunchHeads<128, Bf16Pages>(a, grid, rows32, s);
+    half ? LaunchHeads<128, F16Pages>(a, rows, units, rows32, s)
+         : LaunchHeads<128, Bf16Pages>(a, rows, units, rows32, s);
   else
-    half ? LaunchHeads<64, F16Pages>(a, grid, rows32, s)
-         : LaunchHeads<64, Bf16Pages>(a, grid, rows32, s);
+    half ? LaunchHeads<64, F16Pages>(a, rows, units, rows32, s)
+         : LaunchHeads<64, Bf16Pages>(a, rows, units, rows32, s);
   return HipStatus(hipGetLastError(), "LFM3 paged heads launch");
 }
 

@@ -1,6 +1,7 @@
 """The paged cache's operators at the edges of their types and arguments:
 probabilities far below the largest, scores that leave one slot, evictions of
-sequences that miss pages. Bounds as in paged_util, or derived beside the test."""
+sequences that miss pages, and sizes at the limits of a launch. Bounds as in
+paged_util, or derived beside the test."""
 import ctypes as C
 
 import numpy as np
@@ -204,3 +205,37 @@ def test_evict_drops_slots_on_no_page(shape, kind, dim):
     for s in range(n):
         at, off, _ = P.slots_of(pool, new[s], left[s] + 1)
         assert np.isfinite(gw[at, :, off]).all()
+
+
+def test_heads_of_more_rows_than_a_launch():
+    """Rows up to 2^25: those of 2^24 and more, all but a few of no sequence."""
+    kv, heads, dim, far = 1, 1, 64, (1 << 24) + 3
+    pool, b = seeded(231, kv, 16, dim, F16, [2, 1], [20, 1])
+    b.starts = b.starts + np.uint32(far)
+    b.rows = far + 4
+    pool.upload(), b.upload()
+    rng = np.random.default_rng(232)
+    x = rng.standard_normal((3, dim), np.float32)
+    rows = L.DeviceBuffer(b.rows * dim * 4)
+    out = L.DeviceBuffer(b.rows * dim * 4)
+    rows.upload(x, far * dim * 4)
+    out.upload(np.full((5, dim), 7.0, np.float32), (far - 1) * dim * 4)
+    out.upload(np.full((1, dim), 7.0, np.float32))
+    ones = L.DeviceBuffer.of(np.ones(dim, np.float32))
+    freq = L.DeviceBuffer.of((1e4 ** (-2.0 * np.arange(dim // 2) / dim)).astype(np.float32))
+    L.check(L.lib().lfm3_paged_heads(
+        C.byref(pool.cache), C.byref(b.batch), rows.addr, rows.addr, rows.addr, dim, ones.addr,
+        ones.addr, freq.addr, None, out.addr, dim, F32, heads, 1e-5, None))
+    L.synchronize()
+    near = P.Batch([2, 1], b.lengths, b.table)
+    wq, eq, _, _ = P.heads_rows(near, x[:, None], x[:, None], x[:, None], np.ones(dim),
+                                np.ones(dim), (1e4 ** (-2.0 * np.arange(dim // 2) / dim)
+                                               ).astype(np.float32), None, 1e-5)
+    got = out.download(np.float32, 5 * dim, (far - 1) * dim * 4).reshape(5, 1, dim)
+    assert (got[0] == 7).all() and (got[4] == 7).all()
+    assert (out.download(np.float32, dim) == 7).all()
+    assert (np.abs(got[1:4] - wq) <= eq + np.abs(wq) * 2.0 ** -23).all()
+    _, gv, gw = pool.download()
+    for r, (s, t) in enumerate(((0, 18), (0, 19), (1, 0))):
+        at = (int(b.table[s, t // 16]), 0, t % 16)
+        assert np.array_equal(gv[at], P.to_bits(x[r], F16)) and gw[at] == 0
