@@ -863,8 +863,11 @@ __launch_bounds__(kMergeThreads) __global__ void PagedMergeKernel(AttentionArgs 
   }
 }
 
+// Items of a launch: a grid has less than 2^32 threads in x.
+constexpr std::uint32_t kMaxBlocks = 1u << 22;
+
 template<int D, class T, bool kRows32>
-int LaunchKernels(const AttentionArgs& a, std::uint32_t n_items, hipStream_t s) {
+int LaunchKernels(AttentionArgs a, std::uint32_t n_items, hipStream_t s) {
   constexpr std::size_t kLds = std::size_t(kWaves) * 16384;
   static_assert(kLds >= kStages * 2 * kWideKeys * D * 2, "the wide ring fits");
   static_assert(kLds >= (kWaves * 16 * (D + 4) + 2 * kWaves * 16 + 16) * sizeof(float),
@@ -876,10 +879,19 @@ int LaunchKernels(const AttentionArgs& a, std::uint32_t n_items, hipStream_t s) 
       "LFM3 paged attention shared memory");
   if (e)
     return e;
-  kernel<<<dim3(n_items, kHalves<D, T, kRows32> ? 2 : 1), kThreads, kLds, s>>>(a);
-  if (a.max_records)
-    PagedMergeKernel<D, T, kRows32>
-        <<<dim3(n_items, std::clamp(kMergeBlocks / n_items, 1u, 32u)), kMergeThreads, 0, s>>>(a);
+  const lfm3_paged_item* const items = a.items;
+  for (std::uint32_t at = 0; at < n_items; at += kMaxBlocks) {
+    a.items = items + at;
+    kernel<<<dim3(std::min(n_items - at, kMaxBlocks), kHalves<D, T, kRows32> ? 2 : 1), kThreads,
+             kLds, s>>>(a);
+  }
+  // After every item's records.
+  for (std::uint32_t at = 0; a.max_records && at < n_items; at += kMaxBlocks) {
+    a.items = items + at;
+    PagedMergeKernel<D, T, kRows32><<<dim3(std::min(n_items - at, kMaxBlocks),
+                                           std::clamp(kMergeBlocks / n_items, 1u, 32u)),
+                                      kMergeThreads, 0, s>>>(a);
+  }
   return HipStatus(hipGetLastError(), "LFM3 paged attention launch");
 }
 template<int D, class T>

@@ -239,3 +239,24 @@ def test_heads_of_more_rows_than_a_launch():
     for r, (s, t) in enumerate(((0, 18), (0, 19), (1, 0))):
         at = (int(b.table[s, t // 16]), 0, t % 16)
         assert np.array_equal(gv[at], P.to_bits(x[r], F16)) and gw[at] == 0
+
+
+def test_attention_of_more_items_than_a_launch():
+    """A work list past 2^23 items, whose last ones alone hold work; one tile's
+    spans lie on both sides of 2^23."""
+    kv, heads, dim, room = 2, 8, 64, (1 << 23) + 3
+    pool, b = seeded(241, kv, 16, dim, F16, [1, 20], [900, 20])
+    pool.upload(), b.upload()
+    rng = np.random.default_rng(242)
+    call = P.AttentionCall(pool, b, rng.standard_normal((21, heads, dim), np.float32), heads, 0,
+                           items=P.tiled(b, heads, kv, 0, 16, 128))
+    assert sum(it.parts > 1 for it in call.items) > 8
+    size = C.sizeof(L.PagedItem)
+    items = L.DeviceBuffer(room * size)     # those left zero have no rows
+    items.upload(np.frombuffer(bytes(call.items), np.uint8), (room - len(call.items)) * size)
+    L.check(L.lib().lfm3_paged_attention(
+        C.byref(pool.cache), C.byref(b.batch), items.addr, room, call.q.addr, call.q.ld, None,
+        heads, call.out.addr, call.out.ld, F32, call.lse.addr, heads, 0, call.ws.addr, call.need,
+        None))
+    L.synchronize()
+    P.check_attention(call, "items")
