@@ -540,16 +540,16 @@ __launch_bounds__(kSelectThreads) __global__ void PagedSliceKernel(EvictArgs a, 
 // same for every head; where no count was kept (lists of up to kOneBlock slots)
 // each block adds up the table's pages while its rows are on their way.
 template<int D>
-__launch_bounds__(256) __global__ void PagedMoveKernel(EvictArgs a) {
+__launch_bounds__(256) __global__ void PagedMoveKernel(EvictArgs a, std::uint32_t first) {
   constexpr int S = D / 8, kSlots = 256 / S;
   __shared__ unsigned s_wave[4];
   const int g = blockIdx.y, seq = blockIdx.z, seg = threadIdx.x % S;
   const EvictRange range(a, seq);
   const std::size_t list = std::size_t(seq) * a.kv_heads + g;
   const std::uint32_t most = min(range.length, a.budget);
-  if (blockIdx.x * kSlots >= most)
+  if (first + blockIdx.x * kSlots >= most)
     return;
-  const std::uint32_t to = blockIdx.x * kSlots + threadIdx.x / S;
+  const std::uint32_t to = first + blockIdx.x * kSlots + threadIdx.x / S;
   const std::uint32_t from = a.kept[list * a.budget + min(to, most - 1)];
   const std::uint32_t page = a.table.Page(seq, from), new_page = a.new_table.Page(seq, to);
   // An entry that the list does not have reads some slot or page 0.
@@ -705,11 +705,14 @@ int lfm3_paged_evict(const lfm3_paged_cache* cache, const std::uint32_t* tables,
     PagedSelectKernel<<<dim3(cache->kv_heads, seqs), kSelectThreads, ranks, s>>>(a);
   }
   const std::uint32_t most = std::min(budget, max_length), slots = 256 * 8 / cache->dim;
-  const dim3 grid((most + slots - 1) / slots, cache->kv_heads, seqs);
-  if (cache->dim == 128)
-    PagedMoveKernel<128><<<grid, 256, 0, s>>>(a);
-  else
-    PagedMoveKernel<64><<<grid, 256, 0, s>>>(a);
+  for (std::uint32_t first = 0; first < most; first += kMaxBlocks * slots) {
+    const dim3 grid(std::min((most - first + slots - 1) / slots, kMaxBlocks), cache->kv_heads,
+                    seqs);
+    if (cache->dim == 128)
+      PagedMoveKernel<128><<<grid, 256, 0, s>>>(a, first);
+    else
+      PagedMoveKernel<64><<<grid, 256, 0, s>>>(a, first);
+  }
   return HipStatus(hipGetLastError(), "LFM3 paged eviction launch");
 }
 

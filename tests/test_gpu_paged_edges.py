@@ -260,3 +260,32 @@ def test_attention_of_more_items_than_a_launch():
         None))
     L.synchronize()
     P.check_attention(call, "items")
+
+
+@pytest.mark.parametrize("budget", [1000, (1 << 28) + 5])
+def test_evict_within_bounds_of_many_slots(budget):
+    """Bounds (max_length, the budget) far above the lengths: more blocks to move
+    slots than a launch has."""
+    kv, dim, page, longest = 1, 128, 256, (1 << 28) + 300
+    lengths = [1500, 40]
+    pool = P.Pool(251, 14, kv, page, dim, F16)
+    width = -(-longest // page)
+    table, new = (np.full((2, width), 0xFFFFFFFF, np.uint32) for _ in range(2))
+    order = np.random.default_rng(252).permutation(14).astype(np.uint32)
+    table[0, :6], table[1, 0], new[0, :6], new[1, 0] = order[:6], order[6], order[7:13], order[13]
+    pool.upload()
+    kept, k, v, w = P.evict(pool, table, lengths, new, min(budget, 1500), 3, 20)
+    dt, dn, dl = (L.DeviceBuffer.of(np.asarray(x, np.uint32)) for x in (table, new, lengths))
+    out = L.DeviceBuffer(2 * budget * 4)
+    need = L.lib().lfm3_paged_evict_workspace_bytes(2, kv, budget, longest)
+    ws = L.DeviceBuffer(max(need, 16))
+    L.check(L.lib().lfm3_paged_evict(
+        C.byref(pool.cache), dt.addr, width, dl.addr, 2, longest, dn.addr, width, budget, 3, 20,
+        out.addr, ws.addr, need, None))
+    L.synchronize()
+    for s in range(2):
+        n = len(kept[s][0])
+        got = out.download(np.uint32, n + 1, s * budget * 4)
+        assert np.array_equal(got[:n], kept[s][0]) and got[n] == 0
+    gk, gv, gw = pool.download()
+    assert np.array_equal(gk, k) and np.array_equal(gv, v) and np.array_equal(gw, w)
