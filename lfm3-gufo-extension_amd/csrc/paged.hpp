@@ -36,13 +36,6 @@ struct Bf16Pages {
 
 // Element i of rows that are FP32 (kRows32) or the pages' type.
 template<class T, bool kRows32>
-__device__ __forceinline__ float LoadRow(const void* p, std::size_t i) {
-  if constexpr (kRows32)
-    return static_cast<const float*>(p)[i];
-  else
-    return T::Load(static_cast<const Half*>(p)[i]);
-}
-template<class T, bool kRows32>
 __device__ __forceinline__ void StoreRow(void* p, std::size_t i, float x) {
   if constexpr (kRows32)
     static_cast<float*>(p)[i] = x;
@@ -141,17 +134,9 @@ struct RunPages {
   unsigned id[kRuns];
   // Run `r` (uniform).
   __device__ __forceinline__ unsigned Of(int r) const {
-    static_assert(kRuns == 2 || kRuns == 4 || kRuns == 8, "whole pairs");
-    const auto four = [&](int k) {
-      const unsigned a = r & 1 ? id[k + 1] : id[k], b = r & 1 ? id[k + 3] : id[k + 2];
-      return r & 2 ? b : a;
-    };
-    if constexpr (kRuns == 2)
-      return r & 1 ? id[1] : id[0];
-    else if constexpr (kRuns == 4)
-      return four(0);
-    else
-      return r & 4 ? four(4) : four(0);
+    static_assert(kRuns == 4, "two bits");
+    const unsigned a = r & 1 ? id[1] : id[0], b = r & 1 ? id[3] : id[2];
+    return r & 2 ? b : a;
   }
   // Bit r: run r is on no page.
   __device__ __forceinline__ unsigned Holes(unsigned pages) const {
