@@ -222,7 +222,6 @@ struct Digit {
   int low, bits;
   __device__ __forceinline__ explicit Digit(int d)
       : low(d == 0 ? 21 : d == 1 ? 10 : 0), bits(d == 2 ? 10 : kDigitBits) {}
-  __device__ __forceinline__ unsigned Mask() const { return ((1u << bits) - 1) << low; }
   // The bits of the digits before this one.
   __device__ __forceinline__ unsigned Before() const {
     return low + bits == 32 ? 0u : ~0u << (low + bits);
