@@ -44,12 +44,12 @@ __device__ __forceinline__ float HeadSum(float v) {
   return D == 128 ? SumXor32(v) : v;
 }
 
-// A thread's pair of every unit (query heads, then keys, then values) that
-// its part of a wave walks. The angle is formed and taken into [-pi, pi] in
-// FP64: in FP32 position * frequency alone is off by up to 4e-3 radians at
-// position 131072. A row's units share the angle's sine and cosine. Bound by
-// the launch and two dependent reads before the first store: 8 rows of 24 heads
-// of 128 3.0 us; 519 rows of 48 heads of 64 (9.5 MB) 6.0 us, 1.6 TB/s.
+// A thread's pair of one unit (query heads, then keys, then values), D / 2
+// threads a unit; each forms its own angle and takes it into [-pi, pi] in FP64: in
+// FP32 position * frequency alone is off by up to 4e-3 radians at position 131072.
+// Bound by the launch and two dependent reads before the first store: 8 rows of 24
+// heads of 128 3.0 to 3.3 us; 519 rows of 48 heads of 64 (9.5 MB) 6.0 to 6.4 us,
+// 1.5 TB/s, where a launch (3) and the bytes (2) are 5.
 template<int D, class T, bool kRows32>
 __launch_bounds__(256) __global__ void PagedHeadsKernel(HeadsArgs a) {
   constexpr int P = D / 2, kParts = 256 / P;
@@ -72,33 +72,33 @@ __launch_bounds__(256) __global__ void PagedHeadsKernel(HeadsArgs a) {
   constexpr double kTurn = 6.283185307179586476925;
   float sn, cs;
   sincosf(float(angle - kTurn * rint(angle * (1.0 / kTurn))), &sn, &cs);
-  const int units = a.heads + 2 * a.kv_heads;
-  for (int u = blockIdx.y * kParts + part; u < units; u += gridDim.y * kParts) {
-    const bool is_q = u < a.heads, is_k = !is_q && u < a.heads + a.kv_heads;
-    const int g = is_q ? u : is_k ? u - a.heads : u - a.heads - a.kv_heads;
-    const float* x = (is_q ? a.q : is_k ? a.k : a.v) + row * a.ld + std::size_t(g) * D;
-    const float x0 = x[pair], x1 = x[pair + P];
-    float r0 = x0, r1 = x1;
-    if (is_q || is_k) {
-      const float* w = is_q ? a.q_norm : a.k_norm;
-      const float inv = 1.0f / sqrtf(HeadSum<D>(x0 * x0 + x1 * x1) / float(D) + a.eps);
-      const float y0 = (x0 * inv) * w[pair], y1 = (x1 * inv) * w[pair + P];
-      r0 = y0 * cs - y1 * sn;
-      r1 = y1 * cs + y0 * sn;
-    }
-    if (is_q) {
-      const std::size_t at = row * a.ldq + std::size_t(g) * D + pair;
-      StoreRow<T, kRows32>(a.q_out, at, r0);
-      StoreRow<T, kRows32>(a.q_out, at + P, r1);
-    } else if (stored) {
-      const std::size_t cell =
-          (std::size_t(page) * a.kv_heads + g) * page_slots + (slot & (page_slots - 1));
-      Half* pool = is_k ? a.k_pages : a.v_pages;
-      pool[cell * D + pair] = T::Round(r0);
-      pool[cell * D + pair + P] = T::Round(r1);
-      if (is_k && a.weight && pair == 0)
-        a.weight[cell] = 0.0f;
-    }
+  const int u = blockIdx.y * kParts + part;
+  if (u >= a.heads + 2 * a.kv_heads)
+    return;
+  const bool is_q = u < a.heads, is_k = !is_q && u < a.heads + a.kv_heads;
+  const int g = is_q ? u : is_k ? u - a.heads : u - a.heads - a.kv_heads;
+  const float* x = (is_q ? a.q : is_k ? a.k : a.v) + row * a.ld + std::size_t(g) * D;
+  const float x0 = x[pair], x1 = x[pair + P];
+  float r0 = x0, r1 = x1;
+  if (is_q || is_k) {
+    const float* w = is_q ? a.q_norm : a.k_norm;
+    const float inv = 1.0f / sqrtf(HeadSum<D>(x0 * x0 + x1 * x1) / float(D) + a.eps);
+    const float y0 = (x0 * inv) * w[pair], y1 = (x1 * inv) * w[pair + P];
+    r0 = y0 * cs - y1 * sn;
+    r1 = y1 * cs + y0 * sn;
+  }
+  if (is_q) {
+    const std::size_t at = row * a.ldq + std::size_t(g) * D + pair;
+    StoreRow<T, kRows32>(a.q_out, at, r0);
+    StoreRow<T, kRows32>(a.q_out, at + P, r1);
+  } else if (stored) {
+    const std::size_t cell =
+        (std::size_t(page) * a.kv_heads + g) * page_slots + (slot & (page_slots - 1));
+    Half* pool = is_k ? a.k_pages : a.v_pages;
+    pool[cell * D + pair] = T::Round(r0);
+    pool[cell * D + pair + P] = T::Round(r1);
+    if (is_k && a.weight && pair == 0)
+      a.weight[cell] = 0.0f;
   }
 }
 
@@ -201,7 +201,7 @@ constexpr int kDigitBits = 11, kBins = 1 << kDigitBits;
 // slices of at least kSlice slots, at most kMaxSlices of them, and of twice as
 // many where those are more than the CUs (128 lists of 32,760 slots 79 us, 105 in
 // slices of 4096; 8 of 65,536 36 us, 38 in slices of 8192). With the move, one
-// block and slices: 32 lists of 8190 slots 31 and 39 us, of 16,000 42 and 40, 160
+// block and slices: 32 lists of 8190 slots 32 and 39 us, of 16,000 44 and 40, 160
 // lists of 16,000 47 and 73; 32 of 24,000 53 and 42, 8 of 32,760 57 and 32.
 constexpr std::uint32_t kOneBlock = 16384, kSlice = 4096, kMaxSlices = 32,
                         kCus = 256;
