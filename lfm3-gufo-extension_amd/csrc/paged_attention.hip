@@ -33,8 +33,9 @@
 //   one of K and V; three leave two tiles' loads in flight behind the one at
 //   hand. Bound by the chain of products, softmax and products of a wave, which
 //   two waves a SIMD overlap in part: 512 F16 rows of 16 heads of 128 over 24,576
-//   slots (104 GFLOP) 118 us, 0.88 PFLOP/s, where the matrix cores' loop alone
-//   reaches 2.3.
+//   slots (104 GFLOP) 114 us without the merge, 0.91 PFLOP/s, where the matrix
+//   cores' loop alone reaches 2.3. (That is call after call; the first 10 ms after
+//   an idle card, before the clock has settled, 134 to 145 us.)
 //
 // Split tiles leave a record a (row, head): the unnormalized output, the
 // maximum, the sum and the scale; PagedMergeKernel adds a row's records in
@@ -660,7 +661,8 @@ __device__ __forceinline__ void WideItem(const AttentionArgs& a, const lfm3_page
 // much (96 registers of query parts, 64 of outputs, the scores and the
 // probabilities' three parts), so a tile of more than 128 columns is two blocks
 // of one each: 512 rows of 16 heads over 24,576 slots 256 us, 303 in one. (Over
-// F16 pages, two parts, 215 and 201.)
+// F16 pages, two parts, 215 and 201, though the one spills 79 registers; the kernels
+// of 16-bit rows of 128 dimensions spill 22 and 23.)
 template<int D, class T, bool kRows32>
 constexpr bool kHalves = kRows32 && D == 128 && T::kType == LFM3_TYPE_BF16;
 
